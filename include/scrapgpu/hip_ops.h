@@ -72,7 +72,8 @@ typedef struct scrapgpu_rope_axes_params {
  * second product (y F32: to two terms of F16, 22 bits, or three of BF16, 24 bits). `causal`: the i-th
  * of n new tokens of a request with m keys sees keys 0 .. m - n + i; otherwise it sees all m. A token
  * that sees no key, or that belongs to no request, gets zeros. What a token does not see does not
- * reach its result, whatever its value (NaN included).
+ * reach its result, whatever its value (NaN included); a value of Inf or NaN that it sees does, however
+ * small the weight (a call that meets one where all its tokens see it reads the values twice).
  *
  * SCRAPGPU_OP_ATTENTION_PROMPT: inputs [q (D x Hq x T), k (D x Hk x Tk), v (D x Hk x Tk), q_start
  * (I32, B + 1) and optionally k_start (I32, B + 1; q_start if absent, Tk = T then)], output [y

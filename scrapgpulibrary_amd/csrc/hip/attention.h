@@ -57,26 +57,21 @@ constexpr int padded(int DW) {
 }
 
 // A weight for F32 results, as the sum of terms of the type, each what the ones before leave: two of F16
-// (22 bits), three of BF16 (24; two leave errors of 4e-6 of the result, where f32 sums leave 3e-7). The
-// terms make up kSplit times the weight, which is a little over 1, so that every term is above zero where
-// the weight is (none then turns an infinite value into NaN); the factor is in all weights alike and goes
-// into the sum that divides them. What a weight below 2^-22 of the largest loses in F16 (below 2^-14,
-// lifted) is under 2^-32 of the largest.
+// (22 bits), three of BF16 (24; two leave errors of 4e-6 of the result, where f32 sums leave 3e-7). What a
+// weight below 2^-22 of the largest loses in F16 (below 2^-14, lifted) is under 2^-32 of the largest.
 template <int DT> constexpr int kTerms = DT == F16 ? 2 : 3;
-template <int DT, int N> constexpr float kSplit = N == 1 ? 1.0f : DT == F16 ? 1.0f + 0x1p-16f : 1.0f + 0x1p-12f + 0x1p-20f;
 template <int DT>
 __device__ __forceinline__ void split(float a, float b, uint32_t (&term)[kTerms<DT>]) {
     constexpr uint32_t M = DT == F16 ? 0xFFFFE000u : 0xFFFF0000u;
     const float x = __uint_as_float(__float_as_uint(a) & M), y = __uint_as_float(__float_as_uint(b) & M);
     if constexpr (DT == F16) {
-        const auto u = __builtin_amdgcn_cvt_pkrtz(x, y), v = __builtin_amdgcn_cvt_pkrtz(fmaf(a, kSplit<DT, 2>, -x), fmaf(b, kSplit<DT, 2>, -y));
+        const auto u = __builtin_amdgcn_cvt_pkrtz(x, y), v = __builtin_amdgcn_cvt_pkrtz(a - x, b - y);
         term[0] = __builtin_bit_cast(uint32_t, u);
         term[1] = __builtin_bit_cast(uint32_t, v);
     } else {
         typedef __bf16 pair __attribute__((ext_vector_type(2)));
-        const float r = fmaf(a, 1.0f + 0x1p-12f, -x), t = fmaf(b, 1.0f + 0x1p-12f, -y);
-        const float r2 = r - __uint_as_float(__float_as_uint(r) & M), t2 = t - __uint_as_float(__float_as_uint(t) & M);
-        const pair v = {(__bf16) fmaf(a, 0x1p-20f, r2), (__bf16) fmaf(b, 0x1p-20f, t2)};
+        const float r = a - x, t = b - y;
+        const pair v = {(__bf16) (r - __uint_as_float(__float_as_uint(r) & M)), (__bf16) (t - __uint_as_float(__float_as_uint(t) & M))};
         term[0] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
         term[1] = __builtin_amdgcn_perm(__float_as_uint(t), __float_as_uint(r), 0x07060302u);
         term[2] = __builtin_bit_cast(uint32_t, v);
@@ -158,7 +153,8 @@ __device__ __forceinline__ void store4(uint8_t * row, int d, float a, float b, f
 // Inf and NaN among values that some rows of a step do not see: a weight of 0 times one of them is
 // NaN, which would reach rows that must not know of it. Such steps look through their values first
 // (16 bytes of LDS at a time); where there are any, each row that sees one adds it to its sums by
-// itself, and zero takes its place before the product.
+// itself, and zero takes its place before the product. (Values that all rows see go into the product as
+// they are: see settle.)
 template <int DT>
 __device__ __forceinline__ bool has_nonfinite(u32x4 w) {
     constexpr uint32_t E = DT == F16 ? 0x7C00u : 0x7F80u;
@@ -192,6 +188,51 @@ __device__ __forceinline__ void each_nonfinite(u32x4 w, int at, F add) {
             if ((h & E) != E) continue;
             add(first + i, __uint_as_float((h & 0x8000u) << 16 | 0x7F800000u | ((h & (0x7FFFu & ~E)) != 0 ? 0x400000u : 0)));
         }
+    }
+}
+
+// Seen values that are infinite make a result infinite however small their weight, but a weight, or a
+// term of it, that rounds to 0 makes it NaN. So a wave whose sums hold a NaN goes over the values of its
+// keys once more: the Inf and NaN that a row sees are all that a sum that came out as NaN is made of (where
+// there are none, it stays NaN). Looking through every step's values beforehand would cost every call.
+//
+// Calls add(key, element, value) for those among the values of keys from .. to - 1, at row_of(key).
+template <int DT, int DP, typename P, typename F>
+__device__ __forceinline__ void each_nonfinite_value(int from, int to, int D, P row_of, F add) {
+    constexpr int NC = DP / 8;
+    const int lane = threadIdx.x & 63, c = lane % NC;
+#pragma unroll 1
+    for (int k = from; k < to; k += 64 / NC) {
+        const int key = k + lane / NC;
+        u32x4 v = {0, 0, 0, 0};
+        if (key < to && 8 * c < D) v = *reinterpret_cast<const u32x4 *>(row_of(key) + 16 * c);
+        each_nonfinite<DT>(v, 8 * lane, [&](int e, float x) { add(k + e / DP, e % DP, x); });
+    }
+}
+// o: a lane's sums, N to each of B blocks; each(add): all of the wave's values that are Inf or NaN; index_of(key,
+// element): which of the lane's sums that is (-1: none, or its row does not see the key)
+template <int B, int N, typename V, typename S, typename I>
+__device__ __forceinline__ void settle(V (&o)[B], S each, I index_of) {
+    uint32_t lost[(B * N + 31) / 32] = {}; // a bit for each sum that is NaN
+#pragma unroll
+    for (int j = 0; j < B * N; ++j) {
+        const float x = o[j / N][j % N];
+        lost[j / 32] |= x != x ? 1u << (j % 32) : 0;
+        o[j / N][j % N] = x != x ? 0.0f : x;
+    }
+    each([&](int key, int e, float x) {
+        const int at = index_of(key, e);
+        uint32_t word = lost[0];
+#pragma unroll
+        for (int w = 1; w < (B * N + 31) / 32; ++w) word = at >> 5 == w ? lost[w] : word;
+        const int mine = at >= 0 && (word >> (at & 31) & 1) ? at : -1;
+#pragma unroll
+        for (int j = 0; j < B * N; ++j) o[j / N][j % N] += mine == j ? x : 0.0f;
+    });
+#pragma unroll
+    for (int j = 0; j < B * N; ++j) {
+        const float x = o[j / N][j % N];
+        o[j / N][j % N] = (lost[j / 32] >> (j % 32) & 1) && x == 0.0f ? NAN : x;
     }
 }
 

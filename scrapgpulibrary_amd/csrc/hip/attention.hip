@@ -398,7 +398,29 @@ __global__ __launch_bounds__(256, DW == 256 ? 1 : 2) void k_attention(AttnLaunch
         }
     }
 
-    l = sum_halves(l) * kSplit<DT, NT>;
+    { // (a NaN among the sums: see settle)
+        f32x16 any = o[0];
+#pragma unroll
+        for (int d = 1; d < DB; ++d) any += o[d];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += (any[i] + any[i + 4]) + (any[i + 8] + any[i + 12]);
+        if (__any(sees > 0 && sum != sum)) {
+            const auto row_of = [&](int key) {
+                if constexpr (!PAGED) return vb + (uint64_t) (t.k0 + key) * a.v_s1;
+                const uint64_t page = (uint32_t) min(max(a.table[t.b * a.t_s1 + (key >> a.shift)], 0), a.n_pages - 1);
+                return vb + page * a.v_s3 + (uint64_t) (key & ((1 << a.shift) - 1)) * a.v_s1;
+            };
+            settle<DB, 16>(
+                o, [&](auto add) { each_nonfinite_value<DT, DP>(s0 * BK, min(s1 * BK, t.kv), a.D, row_of, add); },
+                [&](int key, int e) {
+                    const int at = e - 4 * h; // 32 block + 8 (i / 4) + i % 4
+                    return key < sees && at >= 0 && (at & 4) == 0 ? 16 * (at >> 5) + 4 * (at >> 3 & 3) + (at & 3) : -1;
+                });
+        }
+    }
+
+    l = sum_halves(l);
     if (t.pieces > 1) {
         // The pieces of the tile meet in memory: each writes its sums as its lanes hold them (512
         // consecutive bytes a store), the last to arrive adds all in order, for all its waves' rows.

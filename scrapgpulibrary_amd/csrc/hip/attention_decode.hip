@@ -405,6 +405,30 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
             s = next;
         }
 
+        // (a NaN among the sums: see settle)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f32x4 any = o[b][0];
+#pragma unroll
+            for (int d = 1; d < DB; ++d) any += o[b][d];
+            const float sum = (any[0] + any[1]) + (any[2] + any[3]);
+            if (!__any(sees[b] > 0 && sum != sum)) continue;
+            const auto row_of = [&](int key) {
+                const uint64_t page = (uint32_t) min(max(a.table[p.b * a.t_s1 + (key >> a.shift)], 0), a.n_pages - 1);
+                return vb + page * a.v_s3 + (uint64_t) (key & ((1 << a.shift) - 1)) * a.v_s1;
+            };
+            settle<DB, 4>(
+                o[b],
+                [&](auto add) {
+#pragma unroll 1
+                    for (int at = p.s0 + wid; at < p.s1; at += kWaves) each_nonfinite_value<DT, DP>(at * SK, min(at * SK + SK, p.kv), a.D, row_of, add);
+                },
+                [&](int key, int e) {
+                    const int at = e - 4 * part; // 16 block + i
+                    return key < sees[b] && at >= 0 && (at & 12) == 0 ? 4 * (at >> 4) + (at & 3) : -1;
+                });
+        }
+
         // the waves' sums meet in LDS, 16 rows at a time (the lane's number anew: addresses from here on
         // are formed here, and hold no registers through the loop above)
         int tid = threadIdx.x;
@@ -417,7 +441,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
         for (int b = 0; b < NB; ++b) {
             if (r0 + 16 * b >= rows) break;
             __syncthreads();
-            const float lt = sum_row(l[b]) * kSplit<DT, NT>;
+            const float lt = sum_row(l[b]);
 #pragma unroll
             for (int d = 0; d < DB; ++d) *reinterpret_cast<f32x4 *>(sums + (wid * 16 + (tid & 15)) * OS + 16 * d + 4 * (tid >> 4 & 3)) = o[b][d];
             if ((tid & 48) == 0) {

@@ -1,0 +1,81 @@
+"""ATTENTION_PROMPT and ATTENTION_PAGED where values or weights are at the ends of their ranges."""
+import math
+
+import numpy as np
+import pytest
+
+import scrapgpulibrary_amd as sg
+from tests.serving_util import Tensor, free_all, to_bits, values
+from tests.test_gpu_attention import run
+
+pytestmark = pytest.mark.gpu
+
+D = 64
+
+
+def attention(hip, q, k, v, dtype, out, scale, form, hk=1):
+    """The result [n, Hq, D] of one request with q [n, Hq, D] over k, v [m, Hk, D] (the type's bits),
+    causal: `form` "rows" (few rows over pages), "tiles" (pages) or "prompt"."""
+    n, m, page = len(q), len(k), 16
+    tq, y = Tensor(hip, dtype, q.shape).put(q), Tensor(hip, out, q.shape).fill()
+    if form == "prompt":
+        rest = [Tensor(hip, dtype, x.shape).put(x) for x in (k, v)]
+        rest += [Tensor(hip, sg.I32, (2,)).put([0, i]) for i in (n, m)]
+        op, keep = sg.attention_prompt_op(tq.desc, rest[0].desc, rest[1].desc, rest[2].desc, y.desc, scale, k_start=rest[3].desc)
+    else:
+        pages = -(-m // page)
+        rest = []
+        for x in (k, v):
+            c = np.zeros((pages * page,) + x.shape[1:], x.dtype)
+            c[:m] = x
+            c = c.reshape(pages, page, *x.shape[1:]).swapaxes(1, 2)
+            rest.append(Tensor(hip, dtype, c.shape).put(c))
+        rest += [Tensor(hip, sg.I32, (1, pages)).put(np.arange(pages)), Tensor(hip, sg.I32, (2,)).put([0, n]), Tensor(hip, sg.I32, (1,)).put([m])]
+        op, keep = sg.attention_paged_op(tq.desc, *[t.desc for t in rest], y.desc, scale, max_query=n if form == "rows" else 0)
+    run(hip, op)
+    assert ("rows" in sg.last_launch()[0]) == (form == "rows")
+    got = values(out, y.get())
+    free_all(tq, y, *rest)
+    return got
+
+
+def one_hot(dtype, n, heads, scores):
+    """q and k whose scores (scale 1) are `scores` [m] for every row."""
+    q, k = np.zeros((n, heads, D)), np.zeros((len(scores), 1, D))
+    q[..., 3] = 1
+    k[:, 0, 3] = scores
+    return to_bits(dtype, q), to_bits(dtype, k)
+
+
+FORMS = [("rows", 1), ("rows", 4), ("tiles", 80), ("prompt", 80), ("prompt", 1)]
+
+
+@pytest.mark.parametrize("dtype,out", [(sg.F16, sg.F16), (sg.F16, sg.F32), (sg.BF16, sg.BF16), (sg.BF16, sg.F32)], ids=["f16-f16", "f16-f32", "bf16-bf16", "bf16-f32"])
+@pytest.mark.parametrize("form,n", FORMS, ids=[f"{f}-{n}" for f, n in FORMS])
+@pytest.mark.parametrize("heads", [1, 16])
+def test_infinities_of_small_weight(hip, dtype, out, form, n, heads):
+    """A seen infinite value makes the result infinite however small its weight, in the first step, in
+    the last (which holds keys past the end), alone and beside the other sign (NaN there)."""
+    m = 459 + n
+    for less in (10, 20, 40, 80):  # the weights are e^-less of the largest
+        scores = np.zeros(m)
+        v = np.random.default_rng(less).standard_normal((m, 1, D))
+        for j, d, x in ((1, 5, np.inf), (200, 9, -np.inf), (m - n, 13, np.inf), (2, 17, np.inf), (300, 17, -np.inf), (33, 21, np.nan)):
+            scores[j] = -less
+            v[j, 0, d] = x
+        q, k = one_hot(dtype, n, heads, scores)
+        v = to_bits(dtype, v)
+        got = attention(hip, q, k, v, dtype, out, 1.0, form)
+        w = np.exp(scores)
+        seen = np.arange(m) <= m - n + np.arange(n)[:, None]
+        w = np.where(seen, w, 0.0)
+        fine = np.nan_to_num(values(dtype, v)[:, 0], nan=0.0, posinf=0.0, neginf=0.0)
+        want = (w / w.sum(1, keepdims=True)) @ fine
+        want[:, [5, 13]], want[:, 9], want[:, [17, 21]] = np.inf, -np.inf, np.nan
+        want = np.broadcast_to(want[:, None], got.shape)
+        for sign in (1, -1):
+            assert np.array_equal(got == sign * np.inf, want == sign * np.inf)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        # (the weights: rounded once to the type, as its result; sums of 500 f32 terms)
+        few = np.isfinite(want)
+        assert np.max(np.abs(got - want)[few]) < 2 * {sg.F16: 2.0**-10, sg.BF16: 2.0**-7}[dtype]
