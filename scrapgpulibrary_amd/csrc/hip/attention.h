@@ -25,9 +25,10 @@ constexpr float kNoMax = -1e30f; // the running maximum before any key (finite: 
 // and the sums with it, only when it lags by more than kLag (log2).
 constexpr float kLag = 6.0f;
 // What sums relative to one maximum are worth relative to another; never 0, so that infinite sums stay
-// infinite.
+// infinite. What is left of a finite one at least is 2^-149 of it: f32 weights lie that far apart near zero
+// (a select on infinite sums instead: 512 tokens over 6000 beside 15 single ones, 111 -> 123 us).
 __device__ __forceinline__ float decay(float from, float to) {
-    return fmaxf(__builtin_amdgcn_exp2f(from - to), 1e-38f);
+    return fmaxf(__builtin_amdgcn_exp2f(from - to), 0x1p-149f);
 }
 // F16 weights are scaled by 2^8 (with kLag: at most 2^14 of 65504), so that weights down to 2^-22 of
 // the largest stay normal numbers; the scale cancels in the division by the sum. BF16 needs none.

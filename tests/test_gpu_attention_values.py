@@ -79,3 +79,20 @@ def test_infinities_of_small_weight(hip, dtype, out, form, n, heads):
         # (the weights: rounded once to the type, as its result; sums of 500 f32 terms)
         few = np.isfinite(want)
         assert np.max(np.abs(got - want)[few]) < 2 * {sg.F16: 2.0**-10, sg.BF16: 2.0**-7}[dtype]
+
+
+@pytest.mark.parametrize("out", [sg.BF16, sg.F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("form,n", FORMS, ids=[f"{f}-{n}" for f, n in FORMS])
+def test_large_values_that_fade(hip, out, form, n):
+    """A finite value near the type's largest, in a key that a later one outweighs by e^200: nothing of it
+    is left, whether the later key comes in the same wave's steps, in another's or in another piece."""
+    for m, p in ((260, 1), (260, 40), (260, 130), (4000, 2000), (4000, 3900)):
+        scores, v = np.zeros(m), np.zeros((m, 1, D))
+        scores[p] = 200
+        v[3, 0, 5], v[7, 0, 9] = 8.5e37, -3e38
+        v[p, 0, :] = 0.5
+        q, k = one_hot(sg.BF16, n, 3, scores)
+        got = attention(hip, q, k, to_bits(sg.BF16, v), sg.BF16, out, 1.0, form)
+        sees = m - n + np.arange(n) + 1 > p
+        assert sees.any()
+        assert np.max(np.abs(got[sees] - 0.5)) < 2.0**-7, (m, p)
