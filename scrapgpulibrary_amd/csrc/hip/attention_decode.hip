@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
         while (s < p.s1) {
             const int next = s + kWaves;
             const bool more = next < p.s1;
-            const bool masked = (s + 1) * SK > least || r0 + ROWS > rows;
+            const bool masked = (s + 1) * SK > least; // (rows past the last do not count: nobody reads what becomes of them)
             if (a.D < DW) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
