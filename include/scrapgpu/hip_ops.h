@@ -68,8 +68,9 @@ typedef struct scrapgpu_rope_axes_params {
 /* y[:, h, t] = sum_j softmax_j(scale q[:, h, t] . k_j) v_j over the keys that token t sees, head h of
  * Hq reading key head h / (Hq / Hk). q, k, v are F16 or BF16 (one type), y that type or F32; D is a
  * multiple of 8, at most 256; nb0 is the element size, all other strides and offsets multiples of 16
- * bytes. Scores, maxima and sums are f32; the softmax weights are rounded to the inputs' type for the
- * second product (y F32: to two terms of F16, 22 bits, or three of BF16, 24 bits). `causal`: the i-th
+ * bytes. Scores, maxima and sums are f32; for the second product the softmax weights are sums of terms of
+ * the inputs' type: y F32 two of F16 (22 bits) or three of BF16 (24); 16-bit y two where requests have few
+ * new tokens (see max_query), else one, rounded. `causal`: the i-th
  * of n new tokens of a request with m keys sees keys 0 .. m - n + i; otherwise it sees all m. A token
  * that sees no key, or that belongs to no request, gets zeros. What a token does not see does not
  * reach its result, whatever its value (NaN included); a value of Inf or NaN that it sees does, however

@@ -57,25 +57,32 @@ constexpr int padded(int DW) {
     return DW == 96 ? 128 : DW;
 }
 
-// A weight for F32 results, as the sum of terms of the type, each what the ones before leave: two of F16
-// (22 bits), three of BF16 (24; two leave errors of 4e-6 of the result, where f32 sums leave 3e-7). What a
-// weight below 2^-22 of the largest loses in F16 (below 2^-14, lifted) is under 2^-32 of the largest.
+// A weight as the sum of N terms of the type, each what the ones before leave. F32 results: two of F16 (22
+// bits), three of BF16 (24; two leave errors of 4e-6 of the result, where f32 sums leave 3e-7). 16-bit results
+// of few rows: two (BF16: 16 bits). What a weight below 2^-22 of the largest loses in F16 (below 2^-14, lifted)
+// is under 2^-32 of the largest.
 template <int DT> constexpr int kTerms = DT == F16 ? 2 : 3;
-template <int DT>
-__device__ __forceinline__ void split(float a, float b, uint32_t (&term)[kTerms<DT>]) {
+template <int DT, int N>
+__device__ __forceinline__ void split(float a, float b, uint32_t (&term)[N]) {
     constexpr uint32_t M = DT == F16 ? 0xFFFFE000u : 0xFFFF0000u;
     const float x = __uint_as_float(__float_as_uint(a) & M), y = __uint_as_float(__float_as_uint(b) & M);
+    const float r = a - x, t = b - y;
     if constexpr (DT == F16) {
-        const auto u = __builtin_amdgcn_cvt_pkrtz(x, y), v = __builtin_amdgcn_cvt_pkrtz(a - x, b - y);
+        static_assert(N == 2);
+        const auto u = __builtin_amdgcn_cvt_pkrtz(x, y), v = __builtin_amdgcn_cvt_pkrtz(r, t);
         term[0] = __builtin_bit_cast(uint32_t, u);
         term[1] = __builtin_bit_cast(uint32_t, v);
     } else {
         typedef __bf16 pair __attribute__((ext_vector_type(2)));
-        const float r = a - x, t = b - y;
-        const pair v = {(__bf16) (r - __uint_as_float(__float_as_uint(r) & M)), (__bf16) (t - __uint_as_float(__float_as_uint(t) & M))};
         term[0] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
-        term[1] = __builtin_amdgcn_perm(__float_as_uint(t), __float_as_uint(r), 0x07060302u);
-        term[2] = __builtin_bit_cast(uint32_t, v);
+        if constexpr (N == 2) {
+            const pair v = {(__bf16) r, (__bf16) t};
+            term[1] = __builtin_bit_cast(uint32_t, v);
+        } else {
+            const pair v = {(__bf16) (r - __uint_as_float(__float_as_uint(r) & M)), (__bf16) (t - __uint_as_float(__float_as_uint(t) & M))};
+            term[1] = __builtin_amdgcn_perm(__float_as_uint(t), __float_as_uint(r), 0x07060302u);
+            term[2] = __builtin_bit_cast(uint32_t, v);
+        }
     }
 }
 

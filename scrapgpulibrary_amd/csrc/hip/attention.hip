@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256, DW == 256 ? 1 : 2) void k_attention(AttnLaunch
                 total += p0;
                 total += p1;
                 uint32_t term[NT];
-                split<DT>(p0, p1, term);
+                split<DT, NT>(p0, p1, term);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) w[n][e >> 3][e / 2 & 3] = term[n];
             } else {

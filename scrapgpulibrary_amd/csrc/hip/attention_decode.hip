@@ -363,12 +363,8 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t term[NT];
-                    if constexpr (NT == 1) {
-                        term[0] = round2<DT>(x[2 * i], x[2 * i + 1], l[b]);
-                    } else {
-                        l[b] += x[2 * i] + x[2 * i + 1];
-                        split<DT>(x[2 * i], x[2 * i + 1], term);
-                    }
+                    l[b] += x[2 * i] + x[2 * i + 1];
+                    split<DT, NT>(x[2 * i], x[2 * i + 1], term);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) w[b][n][i] = term[n];
                 }
@@ -517,11 +513,12 @@ hipError_t by_dim(const AttnLaunch & a, const AttnShape & s, uint8_t * scratch, 
     return go<DT, 256, 1, NT>(a, s, scratch, arrive, stream);
 }
 
-// 16-bit results: each weight rounded once, as their own rounding is (two terms: 98.3 -> 101 us for two
-// histories of 131071 keys, 32/8 heads of 128)
+// 16-bit results take weights of two terms: few rows wait for memory, and with one the result's error would
+// be 20 to 40% above that of its own rounding (one token over 900, 64 over up to 8000, two over 131071: the same
+// with one term; 64 rows of one request over 60000 keys 105 us with one, 109 with two)
 template <int DT>
 hipError_t by_result(const AttnLaunch & a, const AttnShape & s, uint8_t * scratch, uint32_t * arrive, hipStream_t stream) {
-    return a.out_type == F32 ? by_dim<DT, kTerms<DT>>(a, s, scratch, arrive, stream) : by_dim<DT, 1>(a, s, scratch, arrive, stream);
+    return a.out_type == F32 ? by_dim<DT, kTerms<DT>>(a, s, scratch, arrive, stream) : by_dim<DT, 2>(a, s, scratch, arrive, stream);
 }
 
 } // namespace

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import scrapgpulibrary_amd as sg
+from tests import attention_weights as aw
 from tests.serving_util import Tensor, free_all, to_bits, values
 from tests.test_gpu_attention import run
 
@@ -96,3 +97,46 @@ def test_large_values_that_fade(hip, out, form, n):
         sees = m - n + np.arange(n) + 1 > p
         assert sees.any()
         assert np.max(np.abs(got[sees] - 0.5)) < 2.0**-7, (m, p)
+
+
+def two_keys(hip, dtype, out, form, delta, v):
+    """Requests of one new token over two keys each (see attention_weights): the results [n, 64]."""
+    n, page = len(delta), 16
+    t = n + (100 if form == "tiles" else 0)  # (tokens of one more request, over the first page: so many that tiles run)
+    q = np.zeros((t, 1, D))
+    q[..., 3] = 1
+    k, vals = np.zeros((n, 2, 1, D)), np.zeros((n, 2, 1, D))
+    k[:, 1, 0, 3], vals[:, 1, 0] = -values(dtype, delta), values(dtype, v)
+    tq, y = Tensor(hip, dtype, q.shape).put(to_bits(dtype, q)), Tensor(hip, out, q.shape).fill()
+    starts = np.append(np.arange(n + 1), [t] if t > n else []).astype(np.int32)
+    if form == "prompt":
+        rest = [Tensor(hip, dtype, (2 * n, 1, D)).put(to_bits(dtype, x.reshape(2 * n, 1, D))) for x in (k, vals)]
+        rest += [Tensor(hip, sg.I32, (n + 1,)).put(i) for i in (starts, 2 * starts)]
+        op, keep = sg.attention_prompt_op(tq.desc, rest[0].desc, rest[1].desc, rest[2].desc, y.desc, 1.0, k_start=rest[3].desc)
+    else:
+        rest = []
+        for x in (k, vals):
+            c = np.zeros((n, 1, page, D))
+            c[:, 0, :2] = x[:, :, 0]
+            rest.append(Tensor(hip, dtype, c.shape).put(to_bits(dtype, c)))
+        b = len(starts) - 1
+        rest += [Tensor(hip, sg.I32, (b, 1)).put(np.arange(b).reshape(b, 1) % n), Tensor(hip, sg.I32, (b + 1,)).put(starts), Tensor(hip, sg.I32, (b,)).put(np.full(b, 2))]
+        op, keep = sg.attention_paged_op(tq.desc, *[x.desc for x in rest], y.desc, 1.0, max_query=1 if form == "rows" else 0)
+    run(hip, op)
+    assert ("rows" in sg.last_launch()[0]) == (form == "rows")
+    got = values(out, y.get())[:n, 0]
+    free_all(tq, y, *rest)
+    return got
+
+
+@pytest.mark.parametrize("dtype,out", [(sg.F16, sg.F16), (sg.F16, sg.F32), (sg.BF16, sg.BF16), (sg.BF16, sg.F32)], ids=["f16-f16", "f16-f32", "bf16-bf16", "bf16-f32"])
+@pytest.mark.parametrize("form", ["rows", "tiles", "prompt"])
+def test_weights_have_the_bits_that_they_should(hip, dtype, out, form):
+    """F32 results: weights of 22 (F16) or 24 bits (BF16). 16-bit results: two terms of the type in the kernel
+    for few rows, one in the tiles."""
+    terms = {sg.F16: 2, sg.BF16: 3}[dtype] if out == sg.F32 else 2 if form == "rows" else 1
+    for seed in range(4):
+        delta, v = aw.inputs(dtype, 64, seed)
+        want = aw.result(dtype, delta, v)
+        over = np.abs(two_keys(hip, dtype, out, form, delta, v) - want) - aw.bound(dtype, out, terms, want)
+        assert np.max(over) <= 0, f"{np.max(over):.3e} over the bound, {np.mean(over > 0):.1%} of the elements"
