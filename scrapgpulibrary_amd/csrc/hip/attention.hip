@@ -40,8 +40,9 @@ struct Work {
 // from the requests' lengths, 64 at a time in each wave. `want` > 0: as many work-groups per key head
 // as the CUs hold; where the longest tile gains by it, the tiles are cut into pieces of one length such
 // that all together make at most about that many (never more than `want` over one for each tile: the
-// `room` of the grid, the sums and the arrival counts); 0: each tile is one piece. False: past the last
-// (the grid's last work-groups, which so delay none: 64 tokens over 6000, 53.9 -> 38.9 us).
+// `room` of the sums and the arrival counts, one less than the grid's); 0: each tile is one piece. False: past
+// the last, as the w.px-th of w.pieces work-groups (w.q0: where the last request's tokens end), or (w.pieces 0) no piece (the grid's last work-groups, which
+// so delay none: 64 tokens over 6000, 53.9 -> 38.9 us).
 template <bool PAGED>
 __device__ __forceinline__ bool find_work(const AttnLaunch & a, int turn, int want, int room, Work & w) {
     const int lane = threadIdx.x & 63;
@@ -116,8 +117,13 @@ __device__ __forceinline__ bool find_work(const AttnLaunch & a, int turn, int wa
         pieces = count_all();
     }
     const int px = pieces - 1 - turn;
-    if (px < 0) return false;
     w.px = px;
+    if (px < 0) {
+        w.q0 = __builtin_amdgcn_readlane(q0 + nq, (a.B - 1) & 63);
+        w.px = turn - pieces;
+        w.pieces = room + 1 - pieces;
+        return false;
+    }
     int base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         int here = pieces;
@@ -144,10 +150,13 @@ __device__ __forceinline__ bool find_work(const AttnLaunch & a, int turn, int wa
             w.pieces = c == 1 ? 1 : max(1, (steps_here + len - 1) / len);
             w.s0 = piece * len;
             w.s1 = min(steps_here, w.s0 + len);
-            return piece < w.pieces;
+            if (piece < w.pieces) return true;
+            w.pieces = 0; // (the tile has fewer steps than pieces)
+            return false;
         }
         base += here;
     }
+    w.pieces = 0;
     return false;
 }
 
@@ -184,13 +193,12 @@ __global__ __launch_bounds__(256, DW == 256 ? 1 : 2) void k_attention(AttnLaunch
 
     // heads next to each other in the grid (work-groups go round the XCDs: with 8 key heads each
     // XCD's L2 holds one head's keys), a sequence's last tiles, which see the most keys, first
-    const int kvh = blockIdx.x % a.Hk, turn = (int) (blockIdx.x / a.Hk) - 1;
-    if (turn < 0) { // (the first work-groups)
-        zero_rest(a, kvh);
+    const int kvh = blockIdx.x % a.Hk, turn = blockIdx.x / a.Hk;
+    Work t;
+    if (!find_work<PAGED>(a, turn, want, (int) (gridDim.x / a.Hk) - 1, t)) {
+        if (t.pieces > 0) zero_rest(a, t.q0, kvh, t.px, t.pieces);
         return;
     }
-    Work t;
-    if (!find_work<PAGED>(a, turn, want, (int) (gridDim.x / a.Hk) - 1, t)) return;
     const int s0 = t.s0, s1 = t.s1;
     // this lane's row, and how many keys it sees
     const int row = t.r0 + 32 * wid + n, tok = row / a.G;
@@ -527,6 +535,9 @@ AttnShape attention_shape(const AttnLaunch & a, int cu_count, bool lean) {
         const int64_t many = (int64_t) ((int64_t) a.B * a.Hk >= 2 * cu_count ? 4 : 2) * cu_count / a.Hk;
         s.want = (int) std::max<int64_t>(0, std::min(std::max<int64_t>(many, 1), fit));
         s.scratch = s.want > 0 ? (size_t) ((s.want + a.B) * piece) : 0; // (no room: requests whole)
+        // work-groups without a piece: one, or what 32 KiB of zeros each ask for
+        const int64_t unused = std::max<int64_t>(0, a.T - (int64_t) a.B * a.max_query), zeros = unused * a.G * a.D * (a.out_type == F32 ? 4 : 2);
+        s.idle = (int) std::max<int64_t>(1, std::min<int64_t>(zeros >> 15, 2 * cu_count / a.Hk));
         return s;
     }
     // Tiles of all requests at most; fewer than the work-groups that the CUs hold at once: the keys may

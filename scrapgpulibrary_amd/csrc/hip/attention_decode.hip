@@ -59,7 +59,9 @@ struct Piece {
 };
 
 // Piece `px` of the pieces of all requests. `want`: pieces wished for in all; 0: one a request. A
-// request of more rows than `limit` (more new tokens than the caller said) is one piece.
+// request of more rows than `limit` (more new tokens than the caller said) is one piece. False: past the
+// last, as the p.first-th of p.count work-groups
+// (p.q0: where the last request's tokens end).
 __device__ __forceinline__ bool find_piece(const AttnLaunch & a, int px, int want, int limit, Piece & p) {
     const int lane = threadIdx.x & 63;
     const auto load = [&](int b, int & q0, int & nq, int & kv, int & steps) {
@@ -114,6 +116,9 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch & a, int px, int wan
         }
         base += __builtin_amdgcn_readlane(sum, min(63, a.B - 1 - b0));
     }
+    p.q0 = __builtin_amdgcn_readlane(q0 + nq, (a.B - 1) & 63);
+    p.first = px - base;
+    p.count = (int) (gridDim.x / a.Hk) - base;
     return false;
 }
 
@@ -204,13 +209,12 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
     const int lane = threadIdx.x & 63;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, part = lane >> 4;
-    const int kvh = blockIdx.x % a.Hk, px = (int) (blockIdx.x / a.Hk) - 1;
-    if (px < 0) {
-        zero_rest(a, kvh);
+    const int kvh = blockIdx.x % a.Hk, px = blockIdx.x / a.Hk;
+    Piece p;
+    if (!find_piece(a, px, want, ROWS, p)) {
+        zero_rest(a, p.q0, kvh, p.first, p.count);
         return;
     }
-    Piece p;
-    if (!find_piece(a, px, want, ROWS, p)) return;
     const int rows = p.nq * a.G;
     const float c = weight_scale(a);
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
@@ -496,7 +500,7 @@ hipError_t go(const AttnLaunch & a, const AttnShape & s, uint8_t * scratch, uint
     const size_t lds = std::max((size_t) kWaves * 2 * SK * 2 * DP, sums);
     const hipError_t e = allow_lds((void *) k_attention_rows<DT, DW, NB, NT>, lds);
     if (e != hipSuccess) return e;
-    const uint64_t grid = (uint64_t) (s.want + a.B + 1) * a.Hk;
+    const uint64_t grid = (uint64_t) (s.want + a.B + s.idle) * a.Hk;
     last_form().grid = grid;
     k_attention_rows<DT, DW, NB, NT><<<dim3((unsigned) grid), dim3(64 * kWaves), lds, stream>>>(a, reinterpret_cast<float *>(scratch), arrive, s.want);
     return hipGetLastError();

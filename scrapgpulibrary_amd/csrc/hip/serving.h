@@ -64,6 +64,7 @@ struct AttnShape {
     int nb;         // few rows: blocks of 16 of them in registers
     int tiles;      // tiles of all requests at most
     int want;       // pieces of all requests' keys (tiles' keys) wished for per key head; 0: none
+    int idle;       // few rows: work-groups to each key head beyond the pieces there can be
     size_t scratch; // bytes
 };
 // `lean`: partial sums within 32 MiB (fewer pieces; results differ in rounding)

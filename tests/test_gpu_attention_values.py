@@ -1,5 +1,6 @@
 """ATTENTION_PROMPT and ATTENTION_PAGED where values or weights are at the ends of their ranges."""
 import math
+import time
 
 import numpy as np
 import pytest
@@ -7,7 +8,7 @@ import pytest
 import scrapgpulibrary_amd as sg
 from tests import attention_weights as aw
 from tests.serving_util import Tensor, free_all, to_bits, values
-from tests.test_gpu_attention import run
+from tests.test_gpu_attention import run, run_paged
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +141,44 @@ def test_weights_have_the_bits_that_they_should(hip, dtype, out, form):
         want = aw.result(dtype, delta, v)
         over = np.abs(two_keys(hip, dtype, out, form, delta, v) - want) - aw.bound(dtype, out, terms, want)
         assert np.max(over) <= 0, f"{np.max(over):.3e} over the bound, {np.mean(over > 0):.1%} of the elements"
+
+
+@pytest.mark.parametrize("form", ["rows", "tiles"])
+@pytest.mark.parametrize("out", [sg.F16, sg.F32], ids=["f16", "f32"])
+@pytest.mark.parametrize("hq,hk,d", [(3, 1, 8), (8, 2, 64), (6, 6, 96), (7, 1, 128), (5, 1, 184), (4, 1, 256)])
+def test_tokens_of_no_request_are_zero(hip, form, out, hq, hk, d):
+    """A fixed batch of which some tokens, or none, live: the others' results are zero, in either kernel."""
+    for reqs, rest in (([(1, 40), (0, 9), (2, 70)], 1), ([(1, 300)], 700), ([(0, 5), (0, 0)], 33), ([(3, 3)] * 70, 250)):
+        run_paged(hip, reqs, hq, hk, d, sg.F16, out, seed=d, rest=rest, max_query=3 if form == "rows" else 0)
+        assert ("rows" in sg.last_launch()[0]) == (form == "rows") or form == "tiles"
+
+
+def test_tokens_of_no_request_cost_little(hip):
+    """64 single tokens in a batch with places for 8192 take less than twice the time of a batch of 64 (their
+    zeros are 64 MiB beside 350 MiB of keys and values)."""
+    dev, st = hip
+    b, kv, page, hk, hq, d = 64, 4096, 16, 8, 32, 128
+    pages = b * kv // page
+    bufs = [dev.alloc(pages * page * hk * d * 2) for _ in range(2)]
+    for buf in bufs:
+        st.write(buf, 0, np.zeros(buf.size, np.uint8))
+    k, v = (sg.tdesc(sg.F16, (d, page, hk, pages), buf) for buf in bufs)
+    table = Tensor(hip, sg.I32, (b, kv // page)).put(np.random.default_rng(1).permutation(pages).reshape(b, -1))
+    starts, lens = Tensor(hip, sg.I32, (b + 1,)).put(np.arange(b + 1)), Tensor(hip, sg.I32, (b,)).put(np.full(b, kv))
+    times = []
+    for t in (b, 8192):
+        q, y = Tensor(hip, sg.F16, (t, hq, d)).put(0), Tensor(hip, sg.F16, (t, hq, d)).fill()
+        op, keep = sg.attention_paged_op(q.desc, k, v, table.desc, starts.desc, lens.desc, y.desc, 0.1, max_query=1)
+        took = []
+        for _ in range(8):
+            at = time.perf_counter()
+            for _ in range(10):
+                st.execute(op)
+            st.sync()
+            took.append(time.perf_counter() - at)
+        times.append(min(took))
+        free_all(q, y)
+    free_all(table, starts, lens)
+    for buf in bufs:
+        buf.free()
+    assert times[1] < 2 * times[0], times
