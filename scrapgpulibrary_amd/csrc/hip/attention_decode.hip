@@ -60,8 +60,7 @@ struct Piece {
 
 // Piece `px` of the pieces of all requests. `want`: pieces wished for in all; 0: one a request. A
 // request of more rows than `limit` (more new tokens than the caller said) is one piece. False: past the
-// last, as the p.first-th of p.count work-groups
-// (p.q0: where the last request's tokens end).
+// last, as the p.first-th of p.count work-groups (p.q0: where the last request's tokens end).
 __device__ __forceinline__ bool find_piece(const AttnLaunch & a, int px, int want, int limit, Piece & p) {
     const int lane = threadIdx.x & 63;
     const auto load = [&](int b, int & q0, int & nq, int & kv, int & steps) {
@@ -82,9 +81,12 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch & a, int px, int wan
         sum_all += (float) n;
     }
     for (int d = 1; d < 64 && d < a.B; d <<= 1) sum_all += __shfl_xor(sum_all, d);
-    const int total = (int) fminf(sum_all * 1.0001f, 1.0e9f) + 1;
-    // (the sum is the same in every lane: said so, the pieces' bounds and all that follows stay scalar)
-    const int per = want == 0 ? 1 << 30 : __builtin_amdgcn_readfirstlane(max(kWaves, (total / want + kWaves) / kWaves * kWaves));
+    // (steps of a piece, so many that there are at most `want` pieces and one more a request, which the grid, the
+    // sums and the arrival counts hold, however long all together are; the sum is the same in every lane: said
+    // so, the pieces' bounds and all that follows stay scalar)
+    const float all = sum_all * 1.0001f;
+    const int share = want == 0 ? 1 << 30 : all < 1.0e9f ? ((int) all + 1) / want : (int) fminf(all / (float) want, 1.0e9f) + 1;
+    const int per = __builtin_amdgcn_readfirstlane(max(kWaves, (share + kWaves) / kWaves * kWaves));
     int base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
         if (b0 > 0) load(b0 + lane, q0, nq, kv, steps);

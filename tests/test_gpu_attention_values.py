@@ -182,3 +182,24 @@ def test_tokens_of_no_request_cost_little(hip):
     for buf in bufs:
         buf.free()
     assert times[1] < 2 * times[0], times
+
+
+def test_more_keys_than_a_whole_number_counts(hip):
+    """40 requests of 2^30 keys each (all in one page, which their tables repeat): 1.3e9 steps of 32 keys in
+    pieces that must not be more than the launch has room for. All scores are 0 and every sum is a whole
+    number that f32 holds, so each result is the mean of the page's values; the next call is right as well."""
+    dev, st = hip
+    b, page, d, w = 40, 65536, 8, 16383
+    v = np.zeros((1, 1, page, d), np.float16)
+    for e in range(d):
+        v[0, 0, e :: 4 + e % 4 * 4, e] = 1
+    table = Tensor(hip, sg.I32, (b, w)).put(0)
+    tk, tv = Tensor(hip, sg.F16, v.shape).put(np.zeros_like(v)), Tensor(hip, sg.F16, v.shape).put(v)
+    q, y = Tensor(hip, sg.F16, (b, 1, d)).put(np.ones((b, 1, d), np.float16)), Tensor(hip, sg.F32, (b, 1, d)).fill()
+    starts, lens = Tensor(hip, sg.I32, (b + 1,)).put(np.arange(b + 1)), Tensor(hip, sg.I32, (b,)).put(np.full(b, w * page))
+    run(hip, sg.attention_paged_op(q.desc, tk.desc, tv.desc, table.desc, starts.desc, lens.desc, y.desc, 1.0, max_query=1)[0])
+    assert "rows" in sg.last_launch()[0]
+    # (the waves' and pieces' sums are whole, their joins round)
+    assert np.max(np.abs(y.get() / v.astype(np.float64).mean(2)[0] - 1)) < 2.0**-18
+    free_all(table, tk, tv, q, y, starts, lens)
+    run_paged(hip, [(1, 5000), (1, 3000)], 4, 1, 64, sg.F16, sg.F32, max_query=1)
