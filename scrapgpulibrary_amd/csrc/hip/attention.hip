@@ -490,7 +490,7 @@ hipError_t go(const AttnLaunch & a, const AttnShape & s, uint8_t * scratch, uint
     const size_t lds = (size_t) 4 * BK * 2 * padded(DW);
     const hipError_t e = allow_lds((void *) k_attention<DT, DW, PAGED, OUT32>, lds);
     if (e != hipSuccess) return e;
-    last_form().grid = (uint64_t) (s.tiles + s.want + 1) * a.Hk;
+    last_form().grid = (uint64_t) attention_groups(a, s);
     k_attention<DT, DW, PAGED, OUT32><<<dim3((unsigned) last_form().grid), dim3(256), lds, stream>>>(a, reinterpret_cast<float *>(scratch), arrive, s.want);
     return hipGetLastError();
 }
@@ -552,6 +552,10 @@ AttnShape attention_shape(const AttnLaunch & a, int cu_count, bool lean) {
         s.scratch = s.want > 0 ? (size_t) ((s.tiles + s.want) * a.Hk * item) : 0;
     }
     return s;
+}
+
+int64_t attention_groups(const AttnLaunch & a, const AttnShape & s) {
+    return (s.few ? (int64_t) s.want + a.B + s.idle : (int64_t) s.tiles + s.want + 1) * a.Hk;
 }
 
 hipError_t launch_attention(const AttnLaunch & a, uint8_t * scratch, uint32_t * arrive, int cu_count, bool lean, hipStream_t stream) {

@@ -502,7 +502,7 @@ hipError_t go(const AttnLaunch & a, const AttnShape & s, uint8_t * scratch, uint
     const size_t lds = std::max((size_t) kWaves * 2 * SK * 2 * DP, sums);
     const hipError_t e = allow_lds((void *) k_attention_rows<DT, DW, NB, NT>, lds);
     if (e != hipSuccess) return e;
-    const uint64_t grid = (uint64_t) (s.want + a.B + s.idle) * a.Hk;
+    const uint64_t grid = (uint64_t) attention_groups(a, s);
     last_form().grid = grid;
     k_attention_rows<DT, DW, NB, NT><<<dim3((unsigned) grid), dim3(64 * kWaves), lds, stream>>>(a, reinterpret_cast<float *>(scratch), arrive, s.want);
     return hipGetLastError();

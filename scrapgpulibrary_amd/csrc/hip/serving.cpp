@@ -318,10 +318,9 @@ scrapgpu_status attention_rule(const scrapgpu_op_desc * d, ServingOp * out, cons
     if (!std::isfinite(p->scale)) return fail.bad("attention: the scale must be finite");
     if (!injective(o)) return fail.bad("attention: elements of the output overlap");
     const scrapgpu_status st = all_apart(d, fail);
-    if (st != SCRAPGPU_STATUS_OK || out == nullptr) return st;
-    sgk::AttnLaunch & a = out->attn;
+    if (st != SCRAPGPU_STATUS_OK) return st;
+    sgk::AttnLaunch a;
     std::memset(&a, 0, sizeof(a));
-    out->empty = T == 0;
     a.dtype = q.dtype;
     a.out_type = o.dtype;
     a.q_s1 = q.nb[1];
@@ -339,7 +338,6 @@ scrapgpu_status attention_rule(const scrapgpu_op_desc * d, ServingOp * out, cons
         a.W = (int) W;
         a.shift = shift;
         a.n_pages = (int) sg::dim1(k.ne[3]);
-        put(out, d->inputs[3], "table", &a.table);
     } else {
         a.k_s1 = k.nb[2];
         a.k_s2 = k.nb[1];
@@ -357,12 +355,18 @@ scrapgpu_status attention_rule(const scrapgpu_op_desc * d, ServingOp * out, cons
     a.causal = p->causal != 0;
     a.paged = paged;
     a.max_query = (int) (p->max_query == 0 || p->max_query > (uint32_t) T ? T : p->max_query);
-    put(out, q, "q", &a.q);
-    put(out, k, "k", &a.k);
-    put(out, v, "v", &a.v);
-    put(out, qs, "q_start", &a.q_start);
-    put(out, at, paged ? "kv_len" : "k_start", &a.k_at);
-    put(out, o, "y", &a.o);
+    // (a launch has fewer than 2^32 threads; the number of CUs changes the pieces alone, by a few hundred)
+    if (sgk::attention_groups(a, sgk::attention_shape(a, 256, false)) >= (1 << 24) - 4096) return fail.no("attention: too many requests, tokens or heads");
+    if (out == nullptr) return st;
+    out->attn = a;
+    out->empty = T == 0;
+    put(out, q, "q", &out->attn.q);
+    put(out, k, "k", &out->attn.k);
+    put(out, v, "v", &out->attn.v);
+    if (paged) put(out, d->inputs[3], "table", &out->attn.table);
+    put(out, qs, "q_start", &out->attn.q_start);
+    put(out, at, paged ? "kv_len" : "k_start", &out->attn.k_at);
+    put(out, o, "y", &out->attn.o);
     out->bytes = (double) T * (double) (Hq * D) * (double) (2 + sg::type_size(o.dtype)) + 4.0 * (double) (paged ? 0 : Tk) * (double) (Hk * D);
     return SCRAPGPU_STATUS_OK;
 }

@@ -69,6 +69,7 @@ struct AttnShape {
 };
 // `lean`: partial sums within 32 MiB (fewer pieces; results differ in rounding)
 AttnShape attention_shape(const AttnLaunch & a, int cu_count, bool lean);
+int64_t attention_groups(const AttnLaunch & a, const AttnShape & s); // work-groups of the launch
 hipError_t launch_attention(const AttnLaunch & a, uint8_t * scratch, uint32_t * arrive, int cu_count, bool lean, hipStream_t stream);
 
 } // namespace sgk

@@ -203,3 +203,25 @@ def test_more_keys_than_a_whole_number_counts(hip):
     assert np.max(np.abs(y.get() / v.astype(np.float64).mean(2)[0] - 1)) < 2.0**-18
     free_all(table, tk, tv, q, y, starts, lens)
     run_paged(hip, [(1, 5000), (1, 3000)], 4, 1, 64, sg.F16, sg.F32, max_query=1)
+
+
+def test_launches_too_large_are_refused(hip):
+    """More work-groups than a launch has (2^32 threads) are refused by the rule; the most that fit, and as
+    many tokens where requests have few, are not."""
+    dev, st = hip
+    buf = dev.alloc(256)
+
+    def prompt(b, t, hk):
+        q, i = sg.tdesc(sg.F16, (8, hk, t), buf), sg.tdesc(sg.I32, (b + 1,), buf)
+        return dev.supported(sg.attention_prompt_op(q, q, q, i, sg.tdesc(sg.F16, (8, hk, t)), 1.0)[0])
+
+    def paged(b, t, hk, mq):
+        q, i = sg.tdesc(sg.F16, (8, hk, t), buf), sg.tdesc(sg.I32, (b + 1,), buf)
+        c = sg.tdesc(sg.F16, (8, 16, hk, 4), buf)
+        return dev.supported(sg.attention_paged_op(q, c, c, sg.tdesc(sg.I32, (4, b), buf), i, sg.tdesc(sg.I32, (b,), buf), sg.tdesc(sg.F16, (8, hk, t)), 1.0, max_query=mq)[0])
+
+    for status, why in (prompt(65535, 65535, 256), prompt(1, 1 << 23, 256), prompt(65535, 65535, 65535), paged(65535, 65535, 256, 1)):
+        assert status == sg.UNSUPPORTED and "too many" in why, why
+    for status, why in (prompt(65535, 65535, 250), prompt(1, 1 << 23, 200), paged(60000, 60000, 1, 1), paged(64, (1 << 24) - 1, 16, 1)):
+        assert status == sg.OK, why
+    buf.free()
