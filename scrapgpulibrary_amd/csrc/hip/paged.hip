@@ -351,24 +351,40 @@ hipError_t launch_rope(const RopeLaunch & r, int cu_count, hipStream_t stream) {
     };
     const int V = fits(4) ? 4 : 1;
     const int chunks = r.D / (2 * V), heads = r.Hq + 2 * r.Hk;
-    const int64_t threads = (int64_t) r.T * chunks, blocks = (threads + 255) / 256;
-    if (blocks >= ((int64_t) 1 << 31) || threads >= ((int64_t) 1 << 31)) return hipErrorInvalidValue;
-    // few tokens: the heads over more work-groups, until each CU has four
-    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(heads, 4 * cu_count / blocks));
-    const int per = (int) ((heads + split - 1) / split);
-    const dim3 grid((unsigned) blocks, (unsigned) ((heads + per - 1) / per));
-    std::snprintf(last_form().form, sizeof(last_form().form), "rope v=%d heads=%d", V, per);
-    last_form().grid = (uint64_t) grid.x * grid.y;
-    const auto go = [&](auto kernel) { kernel<<<grid, dim3(256), 0, stream>>>(r, chunks, per); };
-    const auto pick = [&](auto in) {
-        constexpr int IN = decltype(in)::value;
-        if (V == 4) r.adjacent ? go(k_rope<IN, 4, true>) : go(k_rope<IN, 4, false>);
-        else r.adjacent ? go(k_rope<IN, 1, true>) : go(k_rope<IN, 1, false>);
-    };
-    if (r.in_type == F32) pick(std::integral_constant<int, F32>{});
-    else if (r.in_type == F16) pick(std::integral_constant<int, F16>{});
-    else pick(std::integral_constant<int, BF16>{});
-    return hipGetLastError();
+    // a launch for as many tokens as 32-bit thread numbers reach (all but a few calls of many GB)
+    const int most = 0x7FFFFFFF / chunks;
+    last_form().grid = 0;
+    for (int64_t t0 = 0; t0 < r.T; t0 += most) {
+        RopeLaunch part = r;
+        part.T = (int) std::min<int64_t>(most, r.T - t0);
+        part.q += t0 * r.q_s2;
+        part.y += t0 * r.y_s2;
+        part.pos += t0 * r.p_s1;
+        if (r.Hk) {
+            part.k += t0 * r.k_s2;
+            part.v += t0 * r.v_s2;
+            part.slots += t0;
+        }
+        const int64_t blocks = ((int64_t) part.T * chunks + 255) / 256;
+        // few tokens: the heads over more work-groups, until each CU has four
+        const int64_t split = std::max<int64_t>(1, std::min<int64_t>(heads, 4 * cu_count / blocks));
+        const int per = (int) ((heads + split - 1) / split);
+        const dim3 grid((unsigned) blocks, (unsigned) ((heads + per - 1) / per));
+        std::snprintf(last_form().form, sizeof(last_form().form), "rope v=%d heads=%d", V, per);
+        last_form().grid += (uint64_t) grid.x * grid.y;
+        const auto go = [&](auto kernel) { kernel<<<grid, dim3(256), 0, stream>>>(part, chunks, per); };
+        const auto pick = [&](auto in) {
+            constexpr int IN = decltype(in)::value;
+            if (V == 4) r.adjacent ? go(k_rope<IN, 4, true>) : go(k_rope<IN, 4, false>);
+            else r.adjacent ? go(k_rope<IN, 1, true>) : go(k_rope<IN, 1, false>);
+        };
+        if (r.in_type == F32) pick(std::integral_constant<int, F32>{});
+        else if (r.in_type == F16) pick(std::integral_constant<int, F16>{});
+        else pick(std::integral_constant<int, BF16>{});
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 } // namespace sgk
