@@ -73,18 +73,30 @@ bool same(const Desc & a, const Desc & b) {
     return true;
 }
 
-// no byte of a is a byte of b: ranges that do not meet, or [D, H, T] views of one buffer whose
-// tokens lie the same distance apart and whose parts of a token do not meet (q, k, v side by side)
+// No byte of a is a byte of b: ranges that do not meet, or that interleave. Where both repeat over an axis of
+// one stride s, and what is left of each without it (one token, one page) is no longer than s, it is enough that
+// one a is apart from the b at most s after it and from the one before that (q, k, v side by side in each token's
+// row; k and v pages in turn).
 bool apart(const Desc & a, const Desc & b) {
     if (a.buffer == nullptr || a.buffer != b.buffer) return true;
     const uint64_t na = sg::nbytes(a), nb = sg::nbytes(b);
     if (na == 0 || nb == 0 || sg::sat_add(a.offset, na) <= b.offset || sg::sat_add(b.offset, nb) <= a.offset) return true;
-    if (sg::dim1(a.ne[3]) != 1 || sg::dim1(b.ne[3]) != 1 || a.ne[2] <= 1 || b.ne[2] <= 1 || a.nb[2] != b.nb[2] || a.nb[2] == 0) return false;
-    Desc ta = a, tb = b;
-    ta.ne[2] = tb.ne[2] = 1;
-    const uint64_t s = a.nb[2], da = a.offset % s, db = b.offset % s, sa = sg::nbytes(ta), sb = sg::nbytes(tb);
-    const uint64_t ab = (db + s - da) % s; // from a's part of a token to b's next one
-    return sa <= ab && ab + sb <= s;
+    for (int i = 1; i < 4; ++i)
+        for (int j = 1; j < 4; ++j) {
+            const uint64_t s = a.nb[i];
+            if (a.ne[i] <= 1 || b.ne[j] <= 1 || s == 0 || b.nb[j] != s) continue;
+            Desc ta = a, tb = b;
+            ta.ne[i] = tb.ne[j] = 1;
+            if (sg::nbytes(ta) > s || sg::nbytes(tb) > s) continue;
+            // (offsets mod s; s more on both sides for the b before)
+            const uint64_t between = (b.offset % s + s - a.offset % s) % s;
+            ta.offset = s;
+            tb.offset = s + between;
+            if (!apart(ta, tb)) continue;
+            tb.offset = between;
+            if (apart(ta, tb)) return true;
+        }
+    return false;
 }
 
 scrapgpu_status all_apart(const scrapgpu_op_desc * d, const Refusal & fail) {

@@ -33,3 +33,46 @@ def test_more_threads_than_32_bits_count(hip):
         close(values(sg.F16, got), want, mag, sg.F16)
     free_all(pos)
     buf.free()
+
+
+@pytest.mark.parametrize("layout", ["pages", "heads", "places"])
+def test_k_and_v_in_one_buffer(hip, layout):
+    """k and v in turn in one buffer: page by page, head by head inside a page, place by place inside a head, gaps
+    between them untouched. What really overlaps is refused."""
+    dev, st = hip
+    r = np.random.default_rng(3)
+    t, hq, hk, d, page, pages, gap = 40, 4, 2, 64, 16, 5, 16
+    order = {"pages": "pkhsd", "heads": "phksd", "places": "phskd"}[layout]
+    size = {"p": pages, "k": 2, "h": hk, "s": page, "d": d}
+    whole = Tensor(hip, sg.F16, [size[c] for c in order], [gap if c in "ks" else 0 for c in order]).put(0)
+    old = whole.get()
+    step = dict(zip(order, whole.strides))
+    cache = lambda at: sg.tdesc(sg.F16, (d, page, hk, pages), whole.buf, offset=at, nb=[2, step["s"], step["h"], step["p"]])  # noqa: E731
+    x = to_bits(sg.F32, r.standard_normal((t, hq + 2 * hk, d)))
+    parts = np.split(x, [hq, hq + hk], axis=1)
+    q, k, v = (Tensor(hip, sg.F32, p.shape).put(p) for p in parts)
+    y = Tensor(hip, sg.F16, (t, hq, d)).fill()
+    pos, slots = r.integers(0, 5000, (t, 1)).astype(np.int32), r.permutation(pages * page)[:t].astype(np.int32)
+    tp, ts = Tensor(hip, sg.I32, pos.shape).put(pos), Tensor(hip, sg.I32, (t,)).put(slots)
+
+    def op(at):
+        return sg.rope_axes_store_op(q.desc, k.desc, v.desc, tp.desc, ts.desc, y.desc, cache(0), cache(at), d)
+
+    status, why = dev.supported(op(step["k"])[0])
+    assert status == sg.OK, why
+    st.execute(op(step["k"])[0])
+    st.sync()
+    got = whole.get()
+    kc, vc = (np.transpose(c, [order.replace("k", "").index(a) for a in "phsd"]) for c in np.moveaxis(got, order.index("k"), 0))
+    want, mag = turned(values(sg.F32, parts[1]), pos, d, None, 0, 0, 10000.0, 1.0)
+    left = np.ones((pages, page), bool)
+    for i, s in enumerate(slots):
+        close(values(sg.F16, kc[s // page, :, s % page]), want[i], mag[i], sg.F16)
+        assert np.array_equal(vc[s // page, :, s % page], to_bits(sg.F16, parts[2][i]))
+        left[s // page, s % page] = False
+    assert not np.swapaxes(kc, 1, 2)[left].any() and not np.swapaxes(vc, 1, 2)[left].any()
+    assert whole.untouched()
+    for at in (0, 16, step["k"] - 48, step["p"], step["p"] + 16, step["h"], step["s"]):
+        status, why = dev.supported(op(at)[0])
+        assert status == sg.INVALID_ARGUMENT and "overlap" in why, at
+    free_all(whole, q, k, v, y, tp, ts)
