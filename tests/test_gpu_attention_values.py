@@ -7,7 +7,7 @@ import pytest
 
 import scrapgpulibrary_amd as sg
 from tests import attention_weights as aw
-from tests.serving_util import Tensor, free_all, to_bits, values
+from tests.serving_util import Tensor, attend, free_all, to_bits, values
 from tests.test_gpu_attention import run, run_paged
 
 pytestmark = pytest.mark.gpu
@@ -225,3 +225,44 @@ def test_launches_too_large_are_refused(hip):
     for status, why in (prompt(65535, 65535, 250), prompt(1, 1 << 23, 200), paged(60000, 60000, 1, 1), paged(64, (1 << 24) - 1, 16, 1)):
         assert status == sg.OK, why
     buf.free()
+
+
+def test_starts_that_go_back_over_a_long_request(hip):
+    """Starts that cover tokens again and again beside one request of 256000 keys: the tiles are more than the
+    launch has places for, and the long one's would be cut. Nothing but results is written, what is written is the
+    result of a request that has the token (or of two, in parts), and the next call is right."""
+    dev, st = hip
+    r = np.random.default_rng(40)
+    t, hq, page, short, long, again = 512, 16, 4096, 64, 256000, 22
+    w = -(-long // page)
+    kc, vc = (to_bits(sg.F16, r.standard_normal((w, 1, page, D))) for _ in range(2))
+    q = to_bits(sg.F16, r.standard_normal((t, hq, D)))
+    starts = [0, t] * again + [0, 8, t]
+    b = len(starts) - 1
+    lens = [short] * (b - 2) + [long, short]
+    tables = np.tile(np.arange(w, dtype=np.int32), (b, 1))
+    tk, tv, tq = (Tensor(hip, sg.F16, x.shape).put(x) for x in (kc, vc, q))
+    y = Tensor(hip, sg.F32, q.shape, (16, 0, 0), 64).fill()
+    ti, tl, tt = Tensor(hip, sg.I32, (b + 1,)).put(starts), Tensor(hip, sg.I32, (b,)).put(lens), Tensor(hip, sg.I32, tables.shape).put(tables)
+    run(hip, sg.attention_paged_op(tq.desc, tk.desc, tv.desc, tt.desc, ti.desc, tl.desc, y.desc, 0.125, causal=0)[0])
+    form, grid = sg.last_launch()
+    want, room = int(form.split("want=")[1]), grid - 1
+    # the pieces that the requests' lengths ask for, by the kernel's rule for their length
+    tiles = [-(-max(0, n) * hq // 128) for n in np.diff(starts)]
+    steps = [-(-m // 64) for m in lens]
+    per = max(8, sum(n * m for n, m in zip(tiles, steps)) // want + 1)
+    for _ in range(3):
+        n = sum(a * -(-m // per) for a, m in zip(tiles, steps))
+        per = per if n <= want else max(per + 1, per * n // want)
+    assert "tiles" in form and max(steps) > per + 6 and sum(a * -(-m // per) for a, m in zip(tiles, steps)) > room > 0
+    assert y.untouched()
+    got = y.get()
+    of = {}
+    for m in (short, long):
+        k, v = (values(sg.F16, c.reshape(-1, 1, D)[:m]) for c in (kc, vc))
+        of[m] = attend(values(sg.F16, q[:8] if m == long else q), k, v, 0.125, 0)[0]
+    fine = np.isnan(got) | (np.abs(got - of[short]) < 1e-4)
+    fine[:8] |= np.abs(got[:8] - of[long]) < 1e-4
+    assert fine.all() and not np.isnan(got[-8:]).any()
+    free_all(tk, tv, tq, y, ti, tl, tt)
+    run_paged(hip, [(40, 2000), (3, 9)], 4, 1, 64, sg.F16, sg.F32, seed=41)
