@@ -5,7 +5,8 @@
  *
  * The cache. k_cache and v_cache are [D, page_size, Hk, n_pages] tensors (any strides that are
  * multiples of 16 bytes, nb0 the element size). Request b's token j lies in page table[j / page_size, b]
- * at place j % page_size; a "slot" is page * page_size + place. page_size is a power of two.
+ * at place j % page_size; a "slot" is page * page_size + place. page_size is a power of two; ATTENTION_PAGED
+ * reads pages of 16 places or more, the other ops take smaller ones too.
  * Everything the device reads as an index (pages, slots, starts, lengths) is kept inside the tensors
  * by the kernels; what an index out of range does is said at each op.
  *
@@ -26,6 +27,7 @@ extern "C" {
  *            free [1]     how many entries of the pool are free pages
  *   outputs  table [W, B] read and written: entry j of request b is its page j
  *            pool [n]     read and written: entries 0 .. free - 1 are the free pages, the last is taken first
+ *                         (n: all pages that there are; one that comes back to a full pool is lost)
  *            left [2]     free pages after the step; requests that were refused
  *            q_start [B + 1], kv_len [B]   what ATTENTION_PAGED takes: request b's new tokens are
  *                         q_start[b] .. q_start[b + 1], its tokens with them kv_len[b] (0 if it has ended)
@@ -48,8 +50,11 @@ typedef struct scrapgpu_paged_plan_params {
  * the others are copied. axis(i): the first sections[0] pairs follow axis 0, the next sections[1]
  * axis 1 and so on; if `interleaved`, pair i follows axis r = i % A where r > 0 and
  * i < A * sections[r], else axis 0. sections sum to n_dims / 2 (interleaved: are checked against it);
- * all zero is one axis. A is 1 to 4. Angles are exact to 2^-24 of a turn for every 32-bit position.
- * y may be x itself (the same tensor).
+ * all zero is one axis. A is 1 to 4. Angles are exact to 2^-24 of a turn for every 32-bit position
+ * (|scale| at most 8, base at least 1).
+ * y may be x itself (the same tensor). The frequencies run on from axis to axis, as text models with
+ * three axes have them. Image encoders often start them anew for each of A equal sections, theta^(-2Aj / n_dims)
+ * for its j-th pair: that is base = theta^A with the positions of axis a multiplied by theta^a.
  *
  * SCRAPGPU_OP_ROPE_AXES_STORE: inputs [q (D x Hq x T), k (D x Hk x T), v (D x Hk x T), pos, slots
  * (I32, T)], outputs [y (D x Hq x T), k_cache, v_cache]: q and k turned as above, q into y and k with
@@ -75,6 +80,8 @@ typedef struct scrapgpu_rope_axes_params {
  * that sees no key, or that belongs to no request, gets zeros. What a token does not see does not
  * reach its result, whatever its value (NaN included); a value of Inf or NaN that it sees does, however
  * small the weight (a call that meets one where all its tokens see it reads the values twice).
+ * Scores (scale q . k) may be up to 2^24 in magnitude, beyond which f32 tells few of them apart and F16 weights
+ * overflow; BF16 values up to 2^100 for sums of weights and values to stay finite.
  *
  * SCRAPGPU_OP_ATTENTION_PROMPT: inputs [q (D x Hq x T), k (D x Hk x Tk), v (D x Hk x Tk), q_start
  * (I32, B + 1) and optionally k_start (I32, B + 1; q_start if absent, Tk = T then)], output [y

@@ -76,3 +76,26 @@ def test_k_and_v_in_one_buffer(hip, layout):
         status, why = dev.supported(op(at)[0])
         assert status == sg.INVALID_ARGUMENT and "overlap" in why, at
     free_all(whole, q, k, v, y, tp, ts)
+
+
+@pytest.mark.parametrize("axes,d", [(2, 80), (2, 64), (4, 64)])
+@pytest.mark.parametrize("adjacent", [0, 1])
+def test_frequencies_that_start_anew_on_each_axis(hip, axes, d, adjacent):
+    """An image encoder's rotation: each of `axes` equal shares of the pairs has the frequencies theta^(-2j / (d / axes)) of
+    its own axis' position. By this op: base theta^axes, and the positions of axis a times theta^a."""
+    theta, t, heads = 100, 50, 3
+    r = np.random.default_rng(axes)
+    x, pos = to_bits(sg.F32, r.standard_normal((t, heads, d))), r.integers(0, 20 if axes == 4 else 73, (t, axes))
+    tx, y = Tensor(hip, sg.F32, x.shape).put(x), Tensor(hip, sg.F32, x.shape).fill()
+    tp = Tensor(hip, sg.I32, pos.shape).put(pos * theta ** np.arange(axes))
+    share = d // 2 // axes
+    hip[1].execute(sg.rope_axes_op(tx.desc, tp.desc, y.desc, d, [share] * axes, adjacent, base=theta**axes)[0])
+    hip[1].sync()
+    ang = np.concatenate([pos[:, a : a + 1] * float(theta) ** (-2 * np.arange(share) / (d / axes)) for a in range(axes)], 1)[:, None]
+    i, j = (np.arange(0, d, 2), np.arange(1, d, 2)) if adjacent else (np.arange(d // 2), np.arange(d // 2) + d // 2)
+    v = values(sg.F32, x)
+    want, mag = v.copy(), np.zeros_like(v)
+    want[..., i], want[..., j] = v[..., i] * np.cos(ang) - v[..., j] * np.sin(ang), v[..., i] * np.sin(ang) + v[..., j] * np.cos(ang)
+    mag[..., i] = mag[..., j] = np.abs(v[..., i]) + np.abs(v[..., j])
+    close(y.get(), want, mag, sg.F32)
+    free_all(tx, y, tp)
