@@ -57,6 +57,11 @@ constexpr int padded(int DW) {
     return DW == 96 ? 128 : DW;
 }
 
+// the kernel for few rows: work-groups per CU that the registers are held to (NB blocks of 16 rows)
+constexpr int resident(int DP, int NB) {
+    return DP * NB <= 64 ? 4 : DP * NB <= 256 && DP < 256 ? 2 : 1;
+}
+
 // A weight as the sum of N terms of the type, each what the ones before leave. F32 results: two of F16 (22
 // bits), three of BF16 (24; two leave errors of 4e-6 of the result, where f32 sums leave 3e-7). 16-bit results
 // of few rows: two (BF16: 16 bits). What a weight below 2^-22 of the largest loses in F16 (below 2^-14, lifted)

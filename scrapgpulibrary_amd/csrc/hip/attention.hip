@@ -529,10 +529,11 @@ AttnShape attention_shape(const AttnLaunch & a, int cu_count, bool lean) {
         s.nb = longest <= 16 ? 1 : std::min(longest <= 32 ? 2 : 4, most_nb);
         const int64_t piece = (int64_t) 16 * s.nb * (DP + 2) * 4 * a.Hk;
         const int64_t fit = room / piece - a.B;
-        // Two work-groups for each CU, all at once; where the requests alone make that many, twice as
-        // many pieces, which even out unequal histories (64 of up to 8000 keys, 8 heads: 147 -> 138 us;
-        // but 16 of them 43.5 -> 45.4, 2 of 131071 99.5 -> 109).
-        const int64_t many = (int64_t) ((int64_t) a.B * a.Hk >= 2 * cu_count ? 4 : 2) * cu_count / a.Hk;
+        // As many work-groups as the CUs hold at once, two each or one (8 requests of 64 rows of 96 over up to
+        // 20000, 128/2 heads: 58.9 us with one for each CU, 85.7 with two); where the requests alone make two
+        // for each CU, four, which even out unequal histories (64 of up to 8000 keys, 8 heads: 147 -> 138 us,
+        // 64 of up to 6000 of 256 elements 247 -> 232; but 16 of up to 8000 43.5 -> 45.4, 2 of 131071 99.5 -> 109).
+        const int64_t many = (int64_t) ((int64_t) a.B * a.Hk >= 2 * cu_count ? 4 : std::min(2, resident(DP, s.nb))) * cu_count / a.Hk;
         s.want = (int) std::max<int64_t>(0, std::min(std::max<int64_t>(many, 1), fit));
         s.scratch = s.want > 0 ? (size_t) ((s.want + a.B) * piece) : 0; // (no room: requests whole)
         // work-groups without a piece: one, or what 32 KiB of zeros each ask for

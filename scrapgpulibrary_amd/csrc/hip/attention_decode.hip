@@ -190,11 +190,6 @@ __device__ __forceinline__ void join_pieces(const AttnLaunch & a, const float * 
     }
 }
 
-// work-groups per CU that the registers are held to
-constexpr int resident(int DP, int NB) {
-    return DP * NB <= 64 ? 4 : DP * NB <= 256 && DP < 256 ? 2 : 1;
-}
-
 template <int DT, int DW, int NB, int NT>
 __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_attention_rows(AttnLaunch a, float * scratch, uint32_t * arrive, int want) {
     constexpr int DP = padded(DW);     // elements between rows in LDS and memory

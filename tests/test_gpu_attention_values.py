@@ -266,3 +266,11 @@ def test_starts_that_go_back_over_a_long_request(hip):
     assert fine.all() and not np.isnan(got[-8:]).any()
     free_all(tk, tv, tq, y, ti, tl, tt)
     run_paged(hip, [(40, 2000), (3, 9)], 4, 1, 64, sg.F16, sg.F32, seed=41)
+
+
+@pytest.mark.parametrize("d,hq,each", [(128, 4, 2), (64, 64, 2), (128, 64, 1), (96, 40, 1), (256, 2, 1)])
+def test_pieces_follow_what_a_cu_holds(hip, d, hq, each):
+    """Few rows: the keys go in as many pieces as the CUs hold work-groups, two each, or one where 64 rows of
+    more than 64 elements, or heads of 256, fill the registers."""
+    run_paged(hip, [(1, 3000), (1, 100)], hq, 1, d, sg.F16, sg.F16, seed=d, max_query=1)
+    assert int(sg.last_launch()[0].split("want=")[1]) == each * 256
