@@ -207,7 +207,7 @@ template <> struct Elem<BF16> {
     static __device__ __bf16 from(float v) { return (__bf16) v; }
 };
 
-template <typename T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) Pack {
+template <typename T, int N> struct alignas(sizeof(T) * N) Pack {
     T e[N];
 };
 
@@ -338,15 +338,15 @@ int bytes_of(int type) {
 
 hipError_t launch_rope(const RopeLaunch & r, int cu_count, hipStream_t stream) {
     if (r.T < 1 || r.D % 2 != 0 || r.n_dims > 256 || r.n_dims > r.D) return hipErrorInvalidValue;
-    // V pairs a thread: 4 where shape and alignment allow it (8 for 16-bit types, loads of 16 bytes: a
-    // thread then has 8 sines to form; 30000 tokens of 8 heads of 256 in bf16 53 us, but 40 with 4, 5329
-    // of 16 of 80 11.4 for 9.7)
+    // V pairs a thread: 4 where shape and alignment allow it, also for 16-bit types, whose loads are 8 bytes
+    // then (with 8 pairs a thread has 8 sines to form: 30000 tokens of 8 heads of 256 in bf16 40 us, 53 with
+    // 8; 5329 of 16 of 80 9.7, 11.4 with 8)
     const auto fits = [&](int v) {
         if (r.n_dims % (2 * v) != 0 || (r.D - r.n_dims) % (2 * v) != 0) return false;
         uint64_t in = reinterpret_cast<uint64_t>(r.q) | (r.Hq > 1 ? r.q_s1 : 0) | (r.T > 1 ? r.q_s2 : 0);
         uint64_t out = reinterpret_cast<uint64_t>(r.y) | (r.Hq > 1 ? r.y_s1 : 0) | (r.T > 1 ? r.y_s2 : 0);
         if (r.Hk) in |= reinterpret_cast<uint64_t>(r.k) | reinterpret_cast<uint64_t>(r.v) | (r.Hk > 1 ? r.k_s1 | r.v_s1 : 0) | (r.T > 1 ? r.k_s2 | r.v_s2 : 0);
-        return in % (uint64_t) std::min(16, v * bytes_of(r.in_type)) == 0 && out % (uint64_t) std::min(16, v * bytes_of(r.out_type)) == 0;
+        return in % (uint64_t) (v * bytes_of(r.in_type)) == 0 && out % (uint64_t) (v * bytes_of(r.out_type)) == 0;
         // (the caches' strides are multiples of 16 bytes)
     };
     const int V = fits(4) ? 4 : 1;
