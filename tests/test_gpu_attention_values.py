@@ -274,3 +274,23 @@ def test_pieces_follow_what_a_cu_holds(hip, d, hq, each):
     more than 64 elements, or heads of 256, fill the registers."""
     run_paged(hip, [(1, 3000), (1, 100)], hq, 1, d, sg.F16, sg.F16, seed=d, max_query=1)
     assert int(sg.last_launch()[0].split("want=")[1]) == each * 256
+
+
+@pytest.mark.parametrize("dtype,out", [(sg.F16, sg.F16), (sg.F16, sg.F32), (sg.BF16, sg.BF16), (sg.BF16, sg.F32)], ids=["f16-f16", "f16-f32", "bf16-bf16", "bf16-f32"])
+@pytest.mark.parametrize("form,n", FORMS, ids=[f"{f}-{n}" for f, n in FORMS])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_the_largest_magnitude(hip, dtype, out, form, n, sign):
+    """Scores of 2^24 and somewhat less, of either sign, in steps of 2^13 and more: the mean of the values at the
+    largest."""
+    m = 300 + n
+    r = np.random.default_rng(7)
+    q, k, v = np.zeros((n, 2, D)), np.zeros((m, 1, D)), r.integers(-8, 9, (m, 1, D)).astype(float)
+    q[..., 3] = sign * 256
+    k[:, 0, 3] = 65504 - 512 * r.integers(0, 3, m)
+    k, v = to_bits(dtype, k), to_bits(dtype, v)
+    got = attention(hip, to_bits(dtype, q), k, v, dtype, out, 1.0, form)
+    for i in range(n):
+        s = sign * values(dtype, k[: m - n + i + 1, 0, 3])
+        want = values(dtype, v)[: m - n + i + 1, 0][s == s.max()].mean(0)
+        # (equal weights: their rounding cancels; sums of 300 f32 terms of up to 8)
+        assert np.max(np.abs(got[i] - want)) < {sg.F32: 2.0**-18, sg.F16: 2.0**-9, sg.BF16: 2.0**-6}[out]
