@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256, DW == 256 ? 1 : 2) void k_attention(AttnLaunch
     // XCD's L2 holds one head's keys), a sequence's last tiles, which see the most keys, first
     const int kvh = blockIdx.x % a.Hk, turn = blockIdx.x / a.Hk;
     Work t;
-    if (!find_work<PAGED>(a, turn, want, (int) (gridDim.x / a.Hk) - 1, t)) {
+    if (__builtin_expect(!find_work<PAGED>(a, turn, want, (int) (gridDim.x / a.Hk) - 1, t), 0)) {
         if (t.pieces > 0) zero_rest(a, t.q0, kvh, t.px, t.pieces);
         return;
     }
@@ -407,13 +407,11 @@ __global__ __launch_bounds__(256, DW == 256 ? 1 : 2) void k_attention(AttnLaunch
     }
 
     { // (a NaN among the sums: see settle)
-        f32x16 any = o[0];
+        float any[4] = {0.0f, 0.0f, 0.0f, 0.0f}; // (two of them an instruction: a NaN spreads through the products)
 #pragma unroll
-        for (int d = 1; d < DB; ++d) any += o[d];
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += (any[i] + any[i + 4]) + (any[i + 8] + any[i + 12]);
-        if (__any(sees > 0 && sum != sum)) {
+        for (int j = 0; j < DB * 16; j += 2) any[j / 2 & 3] = fmaf(o[j / 16][j % 16], o[j / 16][j % 16 + 1], any[j / 2 & 3]);
+        const float sum = (any[0] + any[1]) + (any[2] + any[3]);
+        if (__builtin_expect(__any(sees > 0 && sum != sum), 0)) {
             const auto row_of = [&](int key) {
                 if constexpr (!PAGED) return vb + (uint64_t) (t.k0 + key) * a.v_s1;
                 const uint64_t page = (uint32_t) min(max(a.table[t.b * a.t_s1 + (key >> a.shift)], 0), a.n_pages - 1);

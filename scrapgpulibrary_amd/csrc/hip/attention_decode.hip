@@ -208,7 +208,7 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
     const int n = lane & 15, part = lane >> 4;
     const int kvh = blockIdx.x % a.Hk, px = blockIdx.x / a.Hk;
     Piece p;
-    if (!find_piece(a, px, want, ROWS, p)) {
+    if (__builtin_expect(!find_piece(a, px, want, ROWS, p), 0)) {
         zero_rest(a, p.q0, kvh, p.first, p.count);
         return;
     }
@@ -405,11 +405,11 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
         // (a NaN among the sums: see settle)
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            f32x4 any = o[b][0];
+            float any[2] = {0.0f, 0.0f}; // (two of them an instruction: a NaN spreads through the products)
 #pragma unroll
-            for (int d = 1; d < DB; ++d) any += o[b][d];
-            const float sum = (any[0] + any[1]) + (any[2] + any[3]);
-            if (!__any(sees[b] > 0 && sum != sum)) continue;
+            for (int j = 0; j < DB * 4; j += 2) any[j / 2 & 1] = fmaf(o[b][j / 4][j % 4], o[b][j / 4][j % 4 + 1], any[j / 2 & 1]);
+            const float sum = any[0] + any[1];
+            if (__builtin_expect(!__any(sees[b] > 0 && sum != sum), 1)) continue;
             const auto row_of = [&](int key) {
                 const uint64_t page = (uint32_t) min(max(a.table[p.b * a.t_s1 + (key >> a.shift)], 0), a.n_pages - 1);
                 return vb + page * a.v_s3 + (uint64_t) (key & ((1 << a.shift) - 1)) * a.v_s1;
