@@ -167,7 +167,7 @@ __device__ __forceinline__ bool find_work(const AttnLaunch & a, int turn, int wa
 //
 // Bound: the matrix units, which are busy 48% of the time, and the softmax between the two products:
 // 64 weights a lane and step. Two work-groups a CU (heads of 128; 3 of 64, 1 of 256) cover one
-// another's softmax and waits. 8192 tokens of 32/8 heads of 128 in bf16: 546 us, 1.01 PFLOP/s, where a
+// another's softmax and waits. 8192 tokens of 32/8 heads of 128 in bf16: 546 to 577 us from card to card, 0.95 to 1.01 PFLOP/s, where a
 // large library product of that type reaches 1.10; F32 results (2 or 3 terms) 0.63 and 0.51 PFLOP/s
 // at 4096 tokens, heads of 256 0.63. Tiles of 256 rows in 8 waves gave 3% at 8192 tokens and lost 11%
 // on packed prompts; a third step on its way through the weights, or no maximum at all, gave nothing.
