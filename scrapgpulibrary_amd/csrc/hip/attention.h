@@ -197,6 +197,12 @@ __device__ __forceinline__ u32x4 only_finite(u32x4 w) {
     for (int i = 0; i < 4; ++i) w[i] = ((w[i] & E) == E ? 0 : w[i] & 0xFFFFu) | ((w[i] & (E << 16)) == (E << 16) ? 0 : w[i] & 0xFFFF0000u);
     return w;
 }
+// the f32 value of 16 bits that are Inf or NaN
+template <int DT>
+__device__ __forceinline__ float nonfinite(uint32_t h) {
+    constexpr uint32_t E = DT == F16 ? 0x7C00u : 0x7F80u;
+    return __uint_as_float((h & 0x8000u) << 16 | 0x7F800000u | ((h & (0x7FFFu & ~E)) != 0 ? 0x400000u : 0));
+}
 // calls add(element, value) for each Inf or NaN of each lane's 16 bytes, one after the other, in all
 // lanes alike; `at`: the lane's first element
 template <int DT, typename F>
@@ -213,7 +219,7 @@ __device__ __forceinline__ void each_nonfinite(u32x4 w, int at, F add) {
         for (int i = 0; i < 8; ++i) {
             const uint32_t h = (i < 2 ? x[0] : i < 4 ? x[1] : i < 6 ? x[2] : x[3]) >> (16 * (i & 1)) & 0xFFFFu;
             if ((h & E) != E) continue;
-            add(first + i, __uint_as_float((h & 0x8000u) << 16 | 0x7F800000u | ((h & (0x7FFFu & ~E)) != 0 ? 0x400000u : 0)));
+            add(first + i, nonfinite<DT>(h));
         }
     }
 }
@@ -223,23 +229,46 @@ __device__ __forceinline__ void each_nonfinite(u32x4 w, int at, F add) {
 // keys once more: the Inf and NaN that a row sees are all that a sum that came out as NaN is made of (where
 // there are none, it stays NaN). Looking through every step's values beforehand would cost every call.
 //
-// Calls add(key, element, value) for those among the values of keys from .. to - 1, at row_of(key).
-template <int DT, int DP, typename P, typename F>
-__device__ __forceinline__ void each_nonfinite_value(int from, int to, int D, P row_of, F add) {
-    constexpr int NC = DP / 8;
-    const int lane = threadIdx.x & 63, c = lane % NC;
+// That is as much work whether a few values are infinite or all: of keys that all rows see, a lane sums
+// the Inf and NaN of its 16 bytes (keys from .. to - 1, at row_of(key)), and the sums go to the rows, add(element, sum).
+template <int DT> struct NonfiniteSum {
+    float sum[8] = {};
+    template <int DP, typename P> __device__ __forceinline__ void take(int from, int to, int D, P row_of) {
+        constexpr int NC = DP / 8;
+        constexpr uint32_t E = DT == F16 ? 0x7C00u : 0x7F80u;
+        const int lane = threadIdx.x & 63, c = lane % NC;
 #pragma unroll 1
-    for (int k = from; k < to; k += 64 / NC) {
-        const int key = k + lane / NC;
-        u32x4 v = {0, 0, 0, 0};
-        if (key < to && 8 * c < D) v = *reinterpret_cast<const u32x4 *>(row_of(key) + 16 * c);
-        each_nonfinite<DT>(v, 8 * lane, [&](int e, float x) { add(k + e / DP, e % DP, x); });
+        for (int k = from; k < to; k += 64 / NC) {
+            const int key = k + lane / NC;
+            u32x4 v = {0, 0, 0, 0};
+            if (key < to && 8 * c < D) v = *reinterpret_cast<const u32x4 *>(row_of(key) + 16 * c);
+            if (!__any(has_nonfinite<DT>(v))) continue;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t h = v[i / 2] >> (16 * (i & 1)) & 0xFFFFu;
+                sum[i] += (h & E) == E ? nonfinite<DT>(h) : 0.0f;
+            }
+        }
     }
-}
-// o: a lane's sums, N to each of B blocks; each(add): all of the wave's values that are Inf or NaN; index_of(key,
-// element): which of the lane's sums that is (-1: none, or its row does not see the key)
-template <int B, int N, typename V, typename S, typename I>
-__device__ __forceinline__ void settle(V (&o)[B], S each, I index_of) {
+    template <int DP, typename F> __device__ __forceinline__ void give(F add) {
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) some |= sum[i] != 0.0f;
+        uint64_t lanes = __ballot(some);
+        while (lanes != 0) {
+            const int l = __builtin_ctzll(lanes);
+            lanes &= lanes - 1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) add(8 * (l % (DP / 8)) + i, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sum[i]), l)));
+        }
+    }
+};
+// o: a lane's sums, N to each of B blocks, fours of them being neighbours: element_of(four) is the first's element,
+// index_of(element) the other way round (-1: not this lane's). below: the values that all rows see; each(visit) calls
+// visit(key) for the keys that some rows do not: each lane looks at its row's own elements there.
+template <int DT, int DP, int B, int N, typename V, typename P, typename S, typename T, typename I>
+__device__ __forceinline__ void settle(V (&o)[B], NonfiniteSum<DT> & below, int sees, int D, P row_of, S each, T element_of, I index_of) {
+    constexpr uint32_t E = DT == F16 ? 0x7C00u : 0x7F80u;
     uint32_t lost[(B * N + 31) / 32] = {}; // a bit for each sum that is NaN
 #pragma unroll
     for (int j = 0; j < B * N; ++j) {
@@ -247,14 +276,31 @@ __device__ __forceinline__ void settle(V (&o)[B], S each, I index_of) {
         lost[j / 32] |= x != x ? 1u << (j % 32) : 0;
         o[j / N][j % N] = x != x ? 0.0f : x;
     }
-    each([&](int key, int e, float x) {
-        const int at = index_of(key, e);
+    below.template give<DP>([&](int e, float x) {
+        const int at = index_of(e);
         uint32_t word = lost[0];
 #pragma unroll
         for (int w = 1; w < (B * N + 31) / 32; ++w) word = at >> 5 == w ? lost[w] : word;
         const int mine = at >= 0 && (word >> (at & 31) & 1) ? at : -1;
 #pragma unroll
         for (int j = 0; j < B * N; ++j) o[j / N][j % N] += mine == j ? x : 0.0f;
+    });
+    each([&](int key) {
+        const uint8_t * row = row_of(key);
+#pragma unroll
+        for (uint32_t & w : lost) asm volatile("" : "+v"(w)); // (else a mask for each bit is kept over the loop)
+#pragma unroll
+        for (int f = 0; f < B * N / 4; ++f) {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            u32x2 v = {0, 0};
+            if (key < sees && element_of(f) < D) v = *reinterpret_cast<const u32x2 *>(row + 2 * element_of(f));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = 4 * f + i;
+                const uint32_t h = v[i / 2] >> (16 * (i & 1)) & 0xFFFFu;
+                o[j / N][j % N] += (h & E) == E && (lost[j / 32] >> (j % 32) & 1) ? nonfinite<DT>(h) : 0.0f;
+            }
+        }
     });
 #pragma unroll
     for (int j = 0; j < B * N; ++j) {

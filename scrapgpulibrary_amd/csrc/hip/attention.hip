@@ -417,11 +417,19 @@ __global__ __launch_bounds__(256, DW == 256 ? 1 : 2) void k_attention(AttnLaunch
                 const uint64_t page = (uint32_t) min(max(a.table[t.b * a.t_s1 + (key >> a.shift)], 0), a.n_pages - 1);
                 return vb + page * a.v_s3 + (uint64_t) (key & ((1 << a.shift) - 1)) * a.v_s1;
             };
-            settle<DB, 16>(
-                o, [&](auto add) { each_nonfinite_value<DT, DP>(s0 * BK, min(s1 * BK, t.kv), a.D, row_of, add); },
-                [&](int key, int e) {
+            const int from = s0 * BK, to = min(s1 * BK, t.kv), apart = max(from, min(to, sees_all));
+            NonfiniteSum<DT> below;
+            below.template take<DP>(from, apart, a.D, row_of);
+            settle<DT, DP, DB, 16>(
+                o, below, sees, a.D, row_of,
+                [&](auto visit) {
+#pragma unroll 1
+                    for (int key = apart; key < to; ++key) visit(key);
+                },
+                [&](int four) { return 32 * (four >> 2) + 8 * (four & 3) + 4 * h; },
+                [&](int e) {
                     const int at = e - 4 * h; // 32 block + 8 (i / 4) + i % 4
-                    return key < sees && at >= 0 && (at & 4) == 0 ? 16 * (at >> 5) + 4 * (at >> 3 & 3) + (at & 3) : -1;
+                    return at >= 0 && (at & 4) == 0 ? 16 * (at >> 5) + 4 * (at >> 3 & 3) + (at & 3) : -1;
                 });
         }
     }

@@ -414,15 +414,21 @@ __global__ __launch_bounds__(64 * kWaves, resident(padded(DW), NB)) void k_atten
                 const uint64_t page = (uint32_t) min(max(a.table[p.b * a.t_s1 + (key >> a.shift)], 0), a.n_pages - 1);
                 return vb + page * a.v_s3 + (uint64_t) (key & ((1 << a.shift) - 1)) * a.v_s1;
             };
-            settle<DB, 4>(
-                o[b],
-                [&](auto add) {
+            NonfiniteSum<DT> below;
 #pragma unroll 1
-                    for (int at = p.s0 + wid; at < p.s1; at += kWaves) each_nonfinite_value<DT, DP>(at * SK, min(at * SK + SK, p.kv), a.D, row_of, add);
+            for (int at = p.s0 + wid; at < p.s1; at += kWaves) below.template take<DP>(at * SK, min(min(at * SK + SK, p.kv), least), a.D, row_of);
+            settle<DT, DP, DB, 4>(
+                o[b], below, sees[b], a.D, row_of,
+                [&](auto visit) {
+#pragma unroll 1
+                    for (int at = p.s0 + wid; at < p.s1; at += kWaves)
+#pragma unroll 1
+                        for (int key = max(at * SK, least); key < min(at * SK + SK, p.kv); ++key) visit(key);
                 },
-                [&](int key, int e) {
+                [&](int four) { return 16 * four + 4 * part; },
+                [&](int e) {
                     const int at = e - 4 * part; // 16 block + i
-                    return key < sees[b] && at >= 0 && (at & 12) == 0 ? 4 * (at >> 4) + (at & 3) : -1;
+                    return at >= 0 && (at & 12) == 0 ? 4 * (at >> 4) + (at & 3) : -1;
                 });
         }
 

@@ -294,3 +294,22 @@ def test_scores_of_the_largest_magnitude(hip, dtype, out, form, n, sign):
         want = values(dtype, v)[: m - n + i + 1, 0][s == s.max()].mean(0)
         # (equal weights: their rounding cancels; sums of 300 f32 terms of up to 8)
         assert np.max(np.abs(got[i] - want)) < {sg.F32: 2.0**-18, sg.F16: 2.0**-9, sg.BF16: 2.0**-6}[out]
+
+
+@pytest.mark.parametrize("form,n", FORMS, ids=[f"{f}-{n}" for f, n in FORMS])
+@pytest.mark.parametrize("d", [64, 72, 256])
+def test_nothing_but_infinities(hip, form, n, d):
+    """All values of many keys infinite, or NaN, or infinite in every other element, with weights that round to zero
+    among them."""
+    m = 1500 + n
+    r = np.random.default_rng(d)
+    q, k = np.zeros((n, 1, d)), np.zeros((m, 1, d))
+    q[..., 3], k[:, 0, 3] = 1, -40 * (r.integers(0, 3, m) > 0)
+    k[100] = 0
+    for i, fill in enumerate((np.inf, -np.inf, np.nan, None)):
+        v = np.full((m, 1, d), fill if fill is not None else 0.25)
+        if fill is None:
+            v[:, :, ::2] = np.inf
+        got = attention(hip, to_bits(sg.F16, q), to_bits(sg.F16, k), to_bits(sg.F16, v), sg.F16, (sg.F16, sg.F32)[i % 2], 1.0, form)
+        want = np.broadcast_to(v[0, 0], got.shape)
+        assert np.array_equal(got, want, equal_nan=True), fill
