@@ -3,8 +3,8 @@
 //
 // Bound: the cache's bytes. All rows of a request that share a key head (new tokens x G heads) are
 // one block of 16 rows, or 2 or 4 of them, so the keys and values of a head are read once. 64 tokens
-// over histories of up to 8000, 32/8 heads of 128: 724 MB in 136 us, 5.3 TB/s; two over 131071: 572 MB
-// in 97.5 us, 5.9 TB/s (reads alone reach 6.45); one over 900: 9.1 us, latency.
+// over histories of up to 8000, 32/8 heads of 128: 724 MB in 135 us, 5.4 TB/s; two over 131071: 572 MB
+// in 97 us, 5.9 TB/s (reads alone reach 6.45); one over 900: 9.2 us, latency.
 //
 // Split. The keys of all requests are cut into pieces of one length, chosen on the device from the
 // requests' lengths so that the pieces of all requests together are about as many as the CUs hold
